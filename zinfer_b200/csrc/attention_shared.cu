@@ -648,8 +648,9 @@ int launch_mma(const SharedArgs& a, cudaStream_t stream) {
 // group's exponentials run while the other loads, stores or waits; the two meet at the end like the chunks of different blocks do.
 // O is rescaled, behind the exponentials, only in warps where a maximum has run 2^8 ahead; warps without a row of the tile only keep
 // the barriers going.  Tiles of 64 or 32 pairs lie in the 128 rows two or four times: each of these PARTS weighs a half or a quarter of a
-// tile's keys (the others' weights are zeros in its rows) relative to a maximum of its own, and they are added up at the end, so that
-// more warps share the exponentials: 6 groups of 9 answers, capped, 33.3 -> 29.1 us.  The sequences' own keys are another kernel's,
+// tile's keys relative to a maximum of its own, and they are added up at the end, so that more warps share the exponentials: 6 groups of
+// 9 answers, capped, 33.3 -> 28.9 us.  P V of a part's keys leaves the lanes of the other parts' rows alone: weights of 0 there would
+// make a NaN of an infinite value.  The sequences' own keys are another kernel's,
 // which runs beside this one: blocks that allocate no tensor memory, in one kernel with those that do, were held back until the others
 // had ended.  Every wait on a barrier is bounded: a block that gives up records a code in *status, stops issuing, frees its tensor
 // memory and returns.
@@ -739,14 +740,6 @@ __device__ __forceinline__ void tmem_put16(unsigned taddr, const float (&v)[16])
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 8 or 16 columns of zeros.
-template <int N>
-__device__ __forceinline__ void tmem_put_zeros(unsigned taddr) {
-  if constexpr (N == 16)
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(taddr), "r"(0) : "memory");
-  else
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(taddr), "r"(0) : "memory");
-}
 __device__ __forceinline__ void tmem_put8(unsigned taddr, const float (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
@@ -866,9 +859,17 @@ __global__ void __maxnreg__(104)
       for (int h = 0; h < ATOMS; ++h) {
         const unsigned long long dv = smem_desc(v_sm + s * TILE + h * BOX);
 #pragma unroll
-        for (int k = 0; k < TK / 16; ++k)   // P: 8 columns (16 keys) further; V: 16 key rows of 128 bytes further
-          umma_bf16_ta(tmem + L::O + (unsigned)(HD * (x & 1) + 64 * h), tmem + L::S + 64u * (unsigned)sb + 8u * (unsigned)k,
-                       dv + (unsigned long long)(128 * k), idesc, (x > 1 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < TK / 16; ++k) {   // P: 8 columns (16 keys) further; V: 16 key rows of 128 bytes further
+          const unsigned to = tmem + L::O + (unsigned)(HD * (x & 1) + 64 * h), from = tmem + L::S + 64u * (unsigned)sb + 8u * (unsigned)k;
+          if constexpr (PARTS == 1) {
+            umma_bf16_ta(to, from, dv + (unsigned long long)(128 * k), idesc, (x > 1 || k > 0) ? 1u : 0u);
+          } else {                            // these keys are one part's: only its rows' lanes take them
+            unsigned off[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) off[i] = 32 * i / PAIRS == 16 * k / NC ? 0u : ~0u;
+            umma_bf16_ta_lanes(to, from, dv + (unsigned long long)(128 * k), idesc, (x > 1 || 16 * k % NC > 0) ? 1u : 0u, off);
+          }
+        }
       }
       umma_commit(&pv_done[sb]);
       umma_commit(&v_empty[s]);
@@ -974,14 +975,11 @@ __global__ void __maxnreg__(104)
             pk[(j - h) / 2] = __uint_as_float(pack_bf16(u.x, u.y));
             pk[(j - h) / 2 + 1] = __uint_as_float(pack_bf16(v.x, v.y));
           }
-          // P lies where its scores lay; the keys of other parts weigh nothing in this row
+          // P lies where its scores lay; under the keys of other parts scores are left, which this row's lane never takes
           const unsigned to = tmem_s + (unsigned)(part * (NC / 2) + h / 2);
           if constexpr (PIECE == 32) tmem_put16(to, pk);
           else tmem_put8(to, pk);
         }
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q)
-          if (q != part) tmem_put_zeros<PARTS == 4 ? 8 : 16>(tmem_s + (unsigned)(q * (NC / 2)));
         l_run += (sum0.x + sum0.y) + (sum1.x + sum1.y);
         tmem_put_wait();
         if (x >= 2 && __any_sync(0xffffffffu, move)) {    // O follows the new maximum once P V of this group's tile before is complete

@@ -69,6 +69,15 @@ __device__ __forceinline__ void umma_bf16_ta(unsigned d_tmem, unsigned a_tmem, u
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same, leaving the lanes of D alone whose bits in off[0] (lanes 0 to 31) .. off[3] are set.
+__device__ __forceinline__ void umma_bf16_ta_lanes(unsigned d_tmem, unsigned a_tmem, unsigned long long b_desc, unsigned idesc,
+                                                   unsigned accumulate, const unsigned (&off)[4]) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
 __device__ __forceinline__ void umma_commit(unsigned long long* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
