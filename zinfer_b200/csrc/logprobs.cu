@@ -68,8 +68,9 @@ __device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w
 __device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 
 // Stands for -inf, and for what lies below it, in the sums: -2^126, a number of both types.  Its weight is 0 like that of -inf, and 0
-// times its difference from any maximum is 0.
-constexpr float LOWEST = -8.507059173023461586e37f;
+// times its difference from a maximum is 0 while that is finite: below 2^127.  From there on the numbers of both types lie 2^103 and more
+// apart, so that whatever is less than the maximum weighs 0, and T, which 0 times an infinite difference may have made a NaN, is 0.
+constexpr float LOWEST = -8.507059173023461586e37f, FAR = 1.7014118346046923173e38f;
 
 // 16 bytes of logits, as they lie in memory until they are used.  `finite` gives the values as the sums take them, for bfloat16
 // two with one maximum.
@@ -454,7 +455,8 @@ __global__ void __launch_bounds__(THREADS, 4)
     if (warp == 0) {
       const float M = warp_max_nan(all.m);
       all.move_to(M);
-      const float S = M > LOWEST ? warp_sum(all.sum()) : NAN, Tt = warp_sum(all.weighted()), norm = logf(S);      // nothing above -inf: NaN
+      const float S = M > LOWEST ? warp_sum(all.sum()) : NAN, norm = logf(S);      // nothing above -inf: NaN
+      const float weighted = warp_sum(all.weighted()), Tt = M >= FAR ? 0.f : weighted;
       ahead = __reduce_add_sync(0xffffffffu, ahead);
       if (lane == 0) {
         logprob[row] = known ? (xt - M) - norm : NAN;
