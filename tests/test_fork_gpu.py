@@ -98,6 +98,23 @@ def test_forks_of_lfm2(model_folders, name, dtype):
             assert helpers.rel_err(got, want) <= 2 * helpers.tol(name, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("head_dim", [256, 258, 320])
+def test_forks_of_heads_wider_than_the_shared_kernels_take(dtype, head_dim):
+    """Heads of more than 256 decode from forks as they do alone: each reads what it shares for itself."""
+    import zinfer_b200 as z
+    cfg = dict(helpers.TINY["loud_a"]["config"], head_dim=head_dim)
+    engine = shared_always(z.Engine(z.random(cfg, seed=3, dtype=dtype, std=0.125), max_batch=4, max_seq_len=128, page_size=16))
+    assert engine._takes_prefixes == (head_dim <= 256)
+    prompt = helpers.random_tokens(7, 70, engine.vocab_size)
+    for decode in (True, False):
+        got, want = forks_and_alone(engine, prompt, 4, 5, 9, decode)
+        assert helpers.rel_err(got, want) <= 2 * helpers.tol("loud_a", dtype)
+    answers, = engine.generate([prompt], max_new_tokens=6, temp=0.0, stop_ids=[], samples=3)
+    alone, = engine.generate([prompt], max_new_tokens=6, temp=0.0, stop_ids=[])
+    assert [len(a.tokens) for a in answers] == [6] * 3 and (dtype == "bfloat16" or all(a.tokens == alone.tokens for a in answers))
+
+
 def test_long_shared_prefix_on_the_tensor_cores(model_folders):
     """More pairs than 32 to a KV head and a prefix over several blocks: the tcgen05 kernel beside the single sequences' one, recorded
     and replayed over the steps at which layouts change, with sequences that end and others among them."""

@@ -109,3 +109,14 @@ def test_the_launcher_refuses_what_it_cannot_copy(views):
     src, dst, _ = k._moves([0], [3], None, 4, 1, "copy")
     desc = np.array(views, dtype=np.int64)
     assert k._fn("cache_copy", "zk_cache_copy")(desc.ctypes.data, 1, src[0], dst[0], None, 1, 1, None) == -22
+
+
+@pytest.mark.parametrize("head_dim,value_dim,scale,takes", [
+    (256, None, None, True), (257, None, None, False), (640, None, None, False), (64, 257, None, False), (320, 64, None, False),
+    (64, None, 0.0, False), (64, None, -0.125, False), (64, None, float("inf"), False), (64, None, float("nan"), False), (64, 256, 2.0, True)])
+def test_attention_takes_prefixes_where_the_kernels_do(head_dim, value_dim, scale, takes):
+    """The layer's rule and the kernels' refusals are one: a step never meets sizes that its kernel turns down."""
+    from zinfer_b200.parts.attention import GqaAttention
+    layer = GqaAttention(64, 4, 2, head_dim, "q", "k", "v", "o", value_dim=value_dim, scale=scale)
+    assert layer.takes_prefixes is takes
+    assert k.attention_shared_takes(layer.run_head_dim, layer.run_value_dim, layer.scale) is takes

@@ -2096,6 +2096,11 @@ def attention_shared_tensor_cores(dtype: torch.dtype, head_dim: int, value_dim: 
     return dtype == torch.bfloat16 and head_dim == value_dim and head_dim in (64, 128) and page_size % 64 == 0
 
 
+def attention_shared_takes(head_dim: int, value_dim: int, scale: float) -> bool:
+    """Whether `attention_shared` has a kernel for heads of these widths and scores of this scale."""
+    return 0 < head_dim <= 256 and 0 < value_dim <= 256 and 0.0 < scale < math.inf
+
+
 def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared: SharedPrefixes, n_heads: int, n_kv: int,
                      head_dim: int, scale: float, longest_own: int, value_dim: Optional[int] = None, softcap: float = 0.0,
                      sink: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
@@ -2121,8 +2126,9 @@ def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, share
                                                  longest_own, value_dim, sink, gate)
     width, front, floats, pages, sizes, launches, _held = call
     _need_here(q, "attention_shared")
-    if not 0.0 < scale < math.inf:
-        raise KernelError(f"attention_shared: a scale of {scale}: positive and finite")
+    if not attention_shared_takes(head_dim, head_dim if value_dim is None else value_dim, scale):
+        raise KernelError(f"attention_shared: keys of {head_dim}, values of {value_dim or head_dim} and a scale of {scale}: heads at most "
+                          "256 wide, and a scale that is positive and finite")
     if status is None:
         status = status_word(q.device)
     else:
@@ -2154,7 +2160,7 @@ def _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n
     _need(page_table, "page_table", torch.int32, (None, None), contiguous=False)
     if page_table.stride(1) != 1:
         raise KernelError("attention_shared: a sequence's page numbers must lie side by side")
-    if n_heads % n_kv or not 0 < head_dim <= 256 or not 0 < vd <= 256:
+    if n_heads % n_kv or not attention_shared_takes(head_dim, vd, 1.0):
         raise KernelError(f"attention_shared: {n_heads} heads on {n_kv}, keys of {head_dim} and values of {vd}: heads must be a "
                           "multiple of the KV heads and at most 256 wide")
     ld_gate = 0

@@ -340,9 +340,10 @@ class GqaAttention(Mixer):
     @property
     def takes_prefixes(self):
         """Whether single-token steps may read what their sequences share once per group: attention over everything before,
-        scores without a bias and weights not mixed across heads."""
+        scores without a bias, weights not mixed across heads, and widths and a scale that the kernels for shared prefixes take."""
         return (self.window <= 0 and self.chunk <= 0 and self.distance_bias is None and self.distance_rows is None
-                and self.talk_name is None)
+                and self.talk_name is None
+                and kernels.attention_shared_takes(self.run_head_dim, self.run_value_dim, self.scale))
 
     # Keys that a step would read over again from which bfloat16 heads of other sizes than the tensor cores' share: their kernel for
     # shared prefixes runs on FMAs, their plain single-token kernel too but leaner (6 heads on 2, 96 wide: 64 sequences behind 1,024
