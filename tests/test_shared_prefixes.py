@@ -120,3 +120,24 @@ def test_attention_takes_prefixes_where_the_kernels_do(head_dim, value_dim, scal
     layer = GqaAttention(64, 4, 2, head_dim, "q", "k", "v", "o", value_dim=value_dim, scale=scale)
     assert layer.takes_prefixes is takes
     assert k.attention_shared_takes(layer.run_head_dim, layer.run_value_dim, layer.scale) is takes
+
+
+@pytest.mark.parametrize("heads,n_kv,width,page,answers,keys,shares", [
+    (32, 8, 32, 64, 64, 2112, False), (8, 8, 32, 64, 64, 8192, False),             # heads of 32: their own kernel is the faster
+    (32, 8, 96, 64, 2, 131136, False), (32, 8, 96, 64, 9, 16448, False), (32, 8, 96, 64, 17, 8256, True), (32, 8, 96, 64, 64, 576, False),
+    (6, 2, 96, 64, 13, 11008, False), (6, 2, 96, 64, 17, 8256, True), (6, 2, 96, 64, 9, 4160, False),
+    (16, 8, 96, 64, 2, 131136, True), (8, 8, 96, 64, 9, 16448, True), (8, 8, 96, 64, 9, 4160, False), (16, 8, 64, 32, 9, 16448, True),
+    (32, 8, 80, 64, 2, 4160, True), (32, 8, 64, 16, 5, 1088, True), (4, 4, 256, 64, 9, 576, True),     # no kernel of their own
+    (32, 8, 64, 64, 5, 1088, True), (8, 8, 128, 64, 2, 4160, True)])                                   # the tensor cores
+def test_bfloat16_heads_share_where_that_is_the_faster(heads, n_kv, width, page, answers, keys, shares):
+    """By the kernel that would otherwise run: times of both are at the rule."""
+    from types import SimpleNamespace
+
+    import torch
+    from zinfer_b200.parts.attention import GqaAttention
+    layer = GqaAttention(64, heads, n_kv, width, "q", "k", "v", "o")
+    ctx = SimpleNamespace(prefixes=k.SharedPrefixes([(range(answers), keys)], answers + 1, "cpu"))
+    kv = SimpleNamespace(page_size=page)
+    assert layer._shares(ctx, kv, torch.bfloat16) is shares
+    assert layer._shares(ctx, kv, torch.float32) is True
+    assert layer._shares(SimpleNamespace(prefixes=None), kv, torch.bfloat16) is False

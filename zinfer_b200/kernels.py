@@ -2004,6 +2004,11 @@ class SharedPrefixes:
         """Keys that a step without sharing reads over again (lengths as rounded for `key`)."""
         return sum((rows - 1) * prefix_capacity(keys) for rows, keys in self.groups)
 
+    @property
+    def read(self) -> int:
+        """Keys of all prefixes, each once (lengths as rounded for `key`)."""
+        return sum(prefix_capacity(keys) for _, keys in self.groups)
+
     @staticmethod
     def word_count(n_seqs: int) -> int:
         return 4 + 4 * (n_seqs // 2) + 2 * n_seqs

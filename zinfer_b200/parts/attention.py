@@ -345,16 +345,30 @@ class GqaAttention(Mixer):
                 and self.talk_name is None
                 and kernels.attention_shared_takes(self.run_head_dim, self.run_value_dim, self.scale))
 
-    # Keys that a step would read over again from which bfloat16 heads of other sizes than the tensor cores' share: their kernel for
-    # shared prefixes runs on FMAs, their plain single-token kernel too but leaner (6 heads on 2, 96 wide: 64 sequences behind 1,024
-    # tokens 31 us against 32, behind 4,096 95 against 47; 8 behind 16,384 49 and 50).
-    general_min_saved = 1 << 17
+    # Where single-token attention of the step's sequences on their own runs on the kernel with a lane per key ("single_token": bfloat16
+    # heads of 32, 64, 96 or 128 that the tensor cores do not take), the shared kernel, on FMAs too but of less speed a pair, pays from so
+    # many keys saved on, and for more than two heads to a KV head from 16 answers a prefix on; heads of 32 it never pays.
+    # Microseconds alone and shared on a B200, 131,072 keys saved: 32 heads on 8, 96 wide, 2 answers 277 and 322, 9 174 and 180, 17 159
+    # and 134, 64 128 and 111; 16 on 8 of 96, 2 answers 320 and 291, 9 150 and 77; 6 on 2 of 96, 13 answers 46 and 51, 17 52 and 41;
+    # 33,280 saved, 9 answers 21 and 26; 32 on 8 of 32, 17 answers 64 and 77, 64 61 and 64.  Every other kernel that attends to one
+    # sequence at a time is the slower from the engine's least saving on: 32 on 8 of 80, 5 answers behind 1,088 tokens 77 and 18, 64
+    # behind 8,192 4,396 and 352; 32 on 8 of 64 in pages of 16 tokens, 5 behind 1,088 64 and 12.
+    general_min_saved, general_min_answers = 1 << 17, 16
 
     def _shares(self, ctx, kv, dtype):
         if ctx.prefixes is None or not self.takes_prefixes:
             return False
-        return (dtype == torch.float32 or kernels.attention_shared_tensor_cores(dtype, self.run_head_dim, self.run_value_dim, kv.page_size)
-                or ctx.prefixes.saved >= self.general_min_saved)
+        if self._plan(dtype, kv.page_size, True)[0] != "single_token":
+            return True
+        saved, read = ctx.prefixes.saved, ctx.prefixes.read
+        return (self.run_head_dim > 32 and saved >= self.general_min_saved
+                and (self.n_heads <= 2 * self.n_kv or saved + read >= self.general_min_answers * read))
+
+    def _plan(self, dtype, page_size, single_token):
+        return kernels.attention_plan(dtype, self.n_heads, self.n_kv, self.run_head_dim, page_size, single_token, self.window,
+                                      self.run_value_dim, self.distance_bias is not None, self.talk_name is not None,
+                                      kept_or_sink=self.keep_first > 0 or self.sink is not None, capped=self.softcap > 0,
+                                      plain_only=self._plain_only)
 
     takes_pending_norm = True
     sums_through_linear = True
@@ -412,11 +426,7 @@ class GqaAttention(Mixer):
 
     def _attend(self, ctx, call, q, qkv):
         kv, hd, vd = call.kv, self.run_head_dim, self.run_value_dim
-        kind, tile_tokens = kernels.attention_plan(q.dtype, self.n_heads, self.n_kv, hd, kv.page_size,
-                                                   ctx.is_decode, self.window, vd,
-                                                   self.distance_bias is not None, self.talk_name is not None,
-                                                   kept_or_sink=self.keep_first > 0 or self.sink is not None,
-                                                   capped=self.softcap > 0, plain_only=self._plain_only)
+        kind, tile_tokens = self._plan(q.dtype, kv.page_size, ctx.is_decode)
         tile_seq, tile_q0 = ctx.memo(("query tiles", tile_tokens), lambda: self._tiles_on_device(ctx, tile_tokens))
         num_splits, split_keys = (key_chunks(ctx.n_seqs, self.n_kv, ctx.max_kv_len, self._sm_count, self.split_keys, self.chunk)
                                   if ctx.is_decode else (1, 0))
