@@ -141,3 +141,17 @@ def test_bfloat16_heads_share_where_that_is_the_faster(heads, n_kv, width, page,
     assert layer._shares(ctx, kv, torch.bfloat16) is shares
     assert layer._shares(ctx, kv, torch.float32) is True
     assert layer._shares(SimpleNamespace(prefixes=None), kv, torch.bfloat16) is False
+
+
+def test_the_tensor_cores_take_what_they_take_without_shared_prefixes():
+    """A fork's weights have as many bits as those of a sequence on its own."""
+    import torch
+    for dtype in (torch.bfloat16, torch.float32):
+        for heads, n_kv in ((16, 8), (16, 1), (17, 1), (32, 2), (34, 2), (64, 1)):
+            for width in (32, 64, 96, 128):
+                for page in (16, 64, 192):
+                    alone = dtype == torch.bfloat16 and bool(k._fn("attention_decode_tc", "zk_attn_decode_tc_takes")(heads, n_kv, width, page))
+                    assert k.attention_shared_tensor_cores(dtype, heads // n_kv, width, width, page) == alone
+                    code = k.dtype_code(dtype)
+                    tile = k._fn("attention_shared", "zk_attn_shared_tile_rows")(code, heads // n_kv, width, width, page, 200, 9000)
+                    assert tile == (128 if alone else 32)

@@ -1268,8 +1268,10 @@ int launch_general(const SharedArgs& a, int tile_rows, cudaStream_t stream) {
   return vec ? launch_general_as<T, 2, true>(a, stream) : launch_general_as<T, 2, false>(a, stream);
 }
 
-static bool mma_takes(int dtype, int hd, int vd, int page_size) {
-  return dtype == ZK_BF16 && hd == vd && (hd == 64 || hd == 128) && page_size % TK == 0;
+// What the tensor cores take: the sizes for which single-token attention without shared prefixes rounds its weights to bfloat16 too.
+// More than 16 heads to a KV head run on float32 FMAs there, and so they do here: a fork's steps are as exact as a sequence's own.
+static bool mma_takes(int dtype, int G, int hd, int vd, int page_size) {
+  return dtype == ZK_BF16 && G <= 16 && hd == vd && (hd == 64 || hd == 128) && page_size % TK == 0;
 }
 
 template <int HD>
@@ -1299,15 +1301,15 @@ int launch_merge(const SharedArgs& a, cudaStream_t stream) {
 extern "C" {
 
 // (sequence, head) pairs that one block's tile of a group holds; `pairs`: the most pairs a group has, `longest`: the keys of the longest
-// prefix.  Tiles of 32, 64 and 128 are the tcgen05 kernel's, tiles of 16 the mma.sync one's (both: bfloat16 heads of 64 or 128 and pages
-// of whole key tiles).  A tile of 16 costs less to start, so it serves groups that fit one, unless their keys are many, and few keys of
-// two (8 KV heads, one group, us): heads of 64, tiles of 16 / 32: 8 pairs behind 1,024 keys 5.9 / 7.5, behind 4,096 9.5 / 8.9, 16
+// prefix.  Tiles of 32, 64 and 128 are the tcgen05 kernel's, tiles of 16 the mma.sync one's (both: bfloat16 heads of 64 or 128, at most
+// 16 to a KV head, and pages of whole key tiles).  A tile of 16 costs less to start, so it serves groups that fit one, unless their keys
+// are many, and few keys of two (8 KV heads, one group, us): heads of 64, tiles of 16 / 32: 8 pairs behind 1,024 keys 5.9 / 7.5, behind 4,096 9.5 / 8.9, 16
 // pairs 6.9 / 7.8, 11.2 / 9.1, 32 behind 256 7.7 / 7.8, behind 1,024 9.1 / 8.3; heads of 128, tiles of 16 / 64: 8 pairs 7.3 / 8.4,
 // 12.0 / 10.1, 16 behind 256 9.3 / 8.2.  Smaller tcgen05 tiles share a row's keys out over more warps: six groups of 32 pairs behind
 // 16,384 keys, tiles of 32 / 64 / 128: heads of 64 40 / 40 / 52, behind 4,096 16.4 / 17.2 / 20.9, of 128 25.9 / 25.4 / 26.5 there.
 // Other types and heads: 32 rows a block on FMAs, 16 where that holds all.
-int zk_attn_shared_tile_rows(int dtype, int hd, int vd, int page_size, int pairs, int longest) {
-  if (!mma_takes(dtype, hd, vd, page_size)) return pairs > 16 ? 32 : 16;
+int zk_attn_shared_tile_rows(int dtype, int G, int hd, int vd, int page_size, int pairs, int longest) {
+  if (!mma_takes(dtype, G, hd, vd, page_size)) return pairs > 16 ? 32 : 16;
   const bool tc5 = hd == 128 ? pairs > 8 || longest >= 4096
                              : longest >= (pairs > 16 ? 1024 : pairs > 8 ? 2048 : 4096) || pairs > 32;
   return !tc5 ? 16 : pairs > 64 ? 128 : pairs > 32 || hd == 128 ? 64 : 32;
@@ -1335,7 +1337,7 @@ int zk_attn_shared(const void* q, const void* k, const void* v, void* out, float
   const SharedArgs a{q, k, v, out, part_o, part_ml, seq_start, seq_slot, page_table, words, sink, gate, status, pt_stride, n, H,
                      Hkv, hd, vd, page_size, ld_gate, scale, softcap, chunk, n_tasks, shared_splits, own_splits, own_keys, H / Hkv,
                      page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), 0};
-  if (mma_takes(dtype, hd, vd, page_size)) {
+  if (mma_takes(dtype, H / Hkv, hd, vd, page_size)) {
     if ((uintptr_t)q % 4 || (uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)out % 8) return ZK_EINVAL;
     const int rc = hd == 64 ? launch_rows<64>(a, tile_rows, num_pages, stream) : launch_rows<128>(a, tile_rows, num_pages, stream);
     if (rc) return rc;

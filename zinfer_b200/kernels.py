@@ -141,7 +141,7 @@ _SIGNATURES = {
     },
     "attention_shared": {
         "zk_attn_shared": "pppppp" + "pppp" + "ppp" + "pffl" + "p",
-        "zk_attn_shared_tile_rows": "iiiiii",
+        "zk_attn_shared_tile_rows": "iiiiiii",
     },
     "cache_copy": {
         "zk_cache_copy": "pipppiip",
@@ -2096,9 +2096,11 @@ def shared_layout(groups: Sequence[tuple], n_seqs: int, group_heads: int, n_kv: 
     return chunk, n_tasks, splits, -(-cap // own_keys), own_keys
 
 
-def attention_shared_tensor_cores(dtype: torch.dtype, head_dim: int, value_dim: int, page_size: int) -> bool:
-    """Whether `attention_shared` runs on the tensor cores for these sizes (else on FMAs)."""
-    return dtype == torch.bfloat16 and head_dim == value_dim and head_dim in (64, 128) and page_size % 64 == 0
+def attention_shared_tensor_cores(dtype: torch.dtype, group_heads: int, head_dim: int, value_dim: int, page_size: int) -> bool:
+    """Whether `attention_shared` runs on the tensor cores, its weights in bfloat16, for `group_heads` heads to a KV head and these
+    sizes (else on float32 FMAs): where `attention` does in a single-token step."""
+    return (dtype == torch.bfloat16 and group_heads <= 16 and head_dim == value_dim and head_dim in (64, 128)
+            and page_size % 64 == 0)
 
 
 def attention_shared_takes(head_dim: int, value_dim: int, scale: float) -> bool:
@@ -2182,8 +2184,8 @@ def _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n
     G, dt = n_heads // n_kv, dtype_code(q.dtype)
     pairs = G * max((rows for rows, _ in shared.groups), default=1)
     longest = max((prefix_capacity(keys) for _, keys in shared.groups), default=0)
-    tile_rows = _fn("attention_shared", "zk_attn_shared_tile_rows")(dt, head_dim, vd, page_size, pairs, longest)
-    fma = not attention_shared_tensor_cores(q.dtype, head_dim, vd, page_size)
+    tile_rows = _fn("attention_shared", "zk_attn_shared_tile_rows")(dt, G, head_dim, vd, page_size, pairs, longest)
+    fma = not attention_shared_tensor_cores(q.dtype, G, head_dim, vd, page_size)
     chunk, n_tasks, splits, own_splits, own_keys = shared.layout(G, n_kv, tile_rows, int(longest_own), sm_count(q.device), fma)
     rows = (splits + own_splits) * n * n_heads
     front = -(-2 * rows // 4) * 4           # (maximum, sum) of every partial result, then the results on 16 bytes
