@@ -882,11 +882,19 @@ __global__ void __maxnreg__(104)
     if (row_ok) pair_of(a, t, pair, b, head);
     {
       constexpr int HALF = HD / 16;      // 16-byte pieces of a row: each group brings one half
-      const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((size_t)b * a.H + head) * HD);
+      const bf16* src = (const bf16*)a.q + ((size_t)b * a.H + head) * HD;
+      const bool whole = (uintptr_t)a.q % 16 == 0;       // else on 4 bytes
 #pragma unroll
       for (int i = 0; i < HALF; ++i) {
         const int ch = wg * HALF + i;
-        *reinterpret_cast<uint4*>(q_sm + (ch / 8) * (T_ROWS * 128) + r * 128 + ((ch ^ r) & 7) * 16) = row_ok ? src[ch] : make_uint4(0, 0, 0, 0);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row_ok && whole) {
+          v = reinterpret_cast<const uint4*>(src)[ch];
+        } else if (row_ok) {
+          const unsigned* w = reinterpret_cast<const unsigned*>(src) + 4 * ch;
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(q_sm + (ch / 8) * (T_ROWS * 128) + r * 128 + ((ch ^ r) & 7) * 16) = v;
       }
       fence_async_smem();
       mbar_arrive(q_full);
@@ -1100,7 +1108,7 @@ int launch_tc5(const SharedArgs& a, long long num_pages, cudaStream_t stream) {
   if (a.n_tasks == 0) return launch_mma<HD>(a, stream);      // nothing is shared
   EncodeTiledFn fn = encode_fn();
   const long long blocks = (long long)a.n_tasks * a.Hkv;
-  if (!fn || blocks > 0x7fffffffLL || !a.status || num_pages <= 0 || (uintptr_t)a.q % 16 || a.chunk % TK) return ZK_EINVAL;
+  if (!fn || blocks > 0x7fffffffLL || !a.status || num_pages <= 0 || a.chunk % TK) return ZK_EINVAL;
   CUtensorMap map[2];
   for (int which = 0; which < 2; ++which) {
     const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)num_pages * a.Hkv * a.page_size};

@@ -2118,7 +2118,8 @@ def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, share
     is laid out.  `softcap`, `sink` and
     `gate` as in `attention`.  `status` (the device's status word unless given) gets 20 where a row is shorter than the prefix it
     shares, 2 where a key has no page.  q [n, H * head_dim],
-    returns [n, H * value_dim], float32 or bfloat16; heads up to 256 wide."""
+    returns [n, H * value_dim], float32 or bfloat16; heads up to 256 wide.  Where the tensor cores run (`attention_shared_tensor_cores`)
+    q lies on 4 bytes and the caches on 16; elsewhere a tensor's own alignment will do."""
     sig = (q.dtype, q.shape, q.is_contiguous(), q.device, k_cache.dtype, k_cache.shape, k_cache.is_contiguous(), k_cache.device,
            v_cache.dtype, v_cache.shape, v_cache.is_contiguous(), v_cache.device, seq_start.dtype, seq_start.shape,
            seq_start.stride(), seq_start.device, seq_slot.dtype, seq_slot.shape, seq_slot.stride(), seq_slot.device, page_table.dtype,
@@ -2131,8 +2132,10 @@ def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, share
             shared._calls.clear()
         call = shared._calls[sig] = _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n_heads, n_kv, head_dim,
                                                  longest_own, value_dim, sink, gate)
-    width, front, floats, pages, sizes, launches, _held = call
+    width, front, floats, pages, sizes, launches, tensor_cores, _held = call
     _need_here(q, "attention_shared")
+    if tensor_cores and (q.data_ptr() % 4 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+        raise KernelError("attention_shared: bfloat16 heads of 64 and 128 need q on 4 bytes and the caches on 16")
     if not attention_shared_takes(head_dim, head_dim if value_dim is None else value_dim, scale):
         raise KernelError(f"attention_shared: keys of {head_dim}, values of {value_dim or head_dim} and a scale of {scale}: heads at most "
                           "256 wide, and a scale that is positive and finite")
@@ -2155,8 +2158,8 @@ def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, share
 def _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n_heads, n_kv, head_dim, longest_own, value_dim, sink,
                  gate) -> tuple:
     """The checks of `attention_shared`'s tensors, and what its launch needs of their sizes: (width of a result row, where the partial
-    results begin behind their maxima and sums, floats of both, pages, the launcher's sizes, how many kernels it launches, and what
-    holds the sizes)."""
+    results begin behind their maxima and sums, floats of both, pages, the launcher's sizes, how many kernels it launches,
+    whether they run on the tensor cores, and what holds the sizes)."""
     _need(q, "q", (torch.float32, torch.bfloat16), (shared.n_seqs, n_heads * head_dim))
     n, vd = q.shape[0], head_dim if value_dim is None else int(value_dim)
     _need(k_cache, "k_cache", q.dtype, (None, n_kv, None, head_dim))
@@ -2191,7 +2194,8 @@ def _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n
     front = -(-2 * rows // 4) * 4           # (maximum, sum) of every partial result, then the results on 16 bytes
     held = array.array("i", (n, n_heads, n_kv, head_dim, vd, page_size, page_table.stride(0), ld_gate, chunk, n_tasks, splits,
                              own_splits, own_keys, tile_rows, dt))
-    return n_heads * vd, front, front + rows * vd, k_cache.shape[0], held.buffer_info()[0], 3 if tile_rows > 16 and not fma and n_tasks else 2, held
+    launches = 3 if tile_rows > 16 and not fma and n_tasks else 2
+    return n_heads * vd, front, front + rows * vd, k_cache.shape[0], held.buffer_info()[0], launches, not fma, held
 
 
 # ------------------------------------------------------------------------------- copies inside the cache
