@@ -287,3 +287,30 @@ def test_log_probabilities_go_to_their_requests():
     assert [r.logprobs for r in results] == [TokenScores([-500.0 * r - 0.5 * k for k in range(3)], [r + 1] * 3, [1.0] * 3) for r in range(3)]
     results = GenerationLoop(Backend(3), 3, 10_000, 1000, 16).run(PROMPTS, Sampler(3), max_new_tokens=3)
     assert all(r.logprobs is None for r in results)
+
+
+class Broken:
+    """Numbers on a device that has failed: reading them raises."""
+
+    def tolist(self):
+        raise RuntimeError("the reader's error")
+
+
+@pytest.mark.parametrize("fails", ["decode", "read_tokens", "token_logprobs"])
+def test_a_step_that_fails_is_what_is_raised(fails):
+    """Log probabilities of the steps before it are not read behind a failure: the step's own error reaches the caller, and the slots
+    are given back."""
+    be, smp = Backend(3), Sampler(3)
+    works, calls = getattr(be, fails), []
+    be.token_logprobs = lambda *args: SimpleNamespace(**dict.fromkeys(("logprob", "rank", "entropy", "top_ids", "top_logprobs"), Broken()))
+
+    def step(*args):
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("the step's error")
+        return (be.__class__.token_logprobs(be, *args) if fails == "token_logprobs" else works(*args))
+
+    setattr(be, fails, step)
+    with pytest.raises(RuntimeError, match="the step's error"):
+        GenerationLoop(be, 3, 10_000, 1000, 16).run(PROMPTS, smp, max_new_tokens=4, logprobs=1)
+    assert sorted(be.free) == [0, 1, 2]

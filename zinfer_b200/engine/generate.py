@@ -201,6 +201,7 @@ class GenerationLoop:
                     self._run_ahead(be, sampler, active, toks, toks_dev, slot_of, out, results, lens, budgets, reasons,
                                     stop, on_step, logprobs, scores)
                     self.stats.t_gen_s += time.perf_counter() - t0
+                    self._tell_scores(scores, results, logprobs)
                     continue
                 while True:
                     live, feed, emitted = [], [], {}
@@ -227,10 +228,9 @@ class GenerationLoop:
                     self.stats.n_decode_steps += 1
                     active = live
                 self.stats.t_gen_s += time.perf_counter() - t0
+                self._tell_scores(scores, results, logprobs)      # (not behind a failure: the device may be what failed)
             finally:
                 be.finish(slots)
-                if scores:
-                    self._tell_scores(scores, results, logprobs)
         return results  # type: ignore[return-value]
 
     @staticmethod
@@ -246,9 +246,9 @@ class GenerationLoop:
 
     @staticmethod
     def _tell_scores(scores, results, top) -> None:
-        """What the steps of a batch left on the device, handed to the requests' results; a request that stopped has been fed one
-        token more than anybody sees."""
-        for requests, rows in scores:
+        """What the steps of a batch left on the device (None: nobody asked for it), handed to the requests' results; a request that
+        stopped has been fed one token more than anybody sees."""
+        for requests, rows in scores or ():
             owners = []
             for r in requests:
                 res = results[r]
