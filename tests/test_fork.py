@@ -314,3 +314,17 @@ def test_a_step_that_fails_is_what_is_raised(fails):
     with pytest.raises(RuntimeError, match="the step's error"):
         GenerationLoop(be, 3, 10_000, 1000, 16).run(PROMPTS, smp, max_new_tokens=4, logprobs=1)
     assert sorted(be.free) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("logprobs", [None, 0, 2])
+def test_requests_that_an_interrupt_keeps_from_running_have_no_log_probabilities_but_the_place_for_them(logprobs):
+    """Every result of a call that asks for them has an entry per token: none for an answer without tokens."""
+    import threading
+    stop = threading.Event()
+    loop = GenerationLoop(Backend(3), 3, 10_000, 1000, 16, interrupt=stop)
+    results = loop.run(PROMPTS, Sampler(6), max_new_tokens=4, samples=2, logprobs=logprobs, on_step=lambda emitted: stop.set())
+    assert [len(r.tokens) for r in results] == [1, 1, 1, 0, 0, 0] and {r.finish_reason for r in results} == {"interrupted"}
+    if logprobs is None:
+        assert all(r.logprobs is None for r in results)
+    else:
+        assert [len(r.logprobs.logprobs) for r in results] == [1, 1, 1, 0, 0, 0]

@@ -164,7 +164,7 @@ class GenerationLoop:
         while pending:
             if self.interrupt.is_set():
                 for r in pending:
-                    results[r] = GenerationResult([], "interrupted", lens[r])
+                    results[r] = GenerationResult([], "interrupted", lens[r], logprobs=None if logprobs is None else TokenScores())
                 break
             batch = plan_batch(pending, lens, budgets, self.max_batch, self.max_tokens, self.page_size)
             pending = pending[len(batch):]
