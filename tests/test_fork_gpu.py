@@ -149,6 +149,49 @@ def test_long_shared_prefix_on_the_tensor_cores(model_folders):
         assert helpers.rel_err(got, want) <= 2 * helpers.tol(name, "bfloat16")
 
 
+@pytest.mark.parametrize("name,dtype,page", [("loud_d", "bf16", 64), ("loud_c", "fp32", 16)])
+def test_steps_of_forks_are_prepared(model_folders, name, dtype, page):
+    """Recorded ahead for sequences that share prefixes, over the lengths at which their launches change, until sharing no longer pays;
+    a batch that has run shared steps alone has none without prefixes to record, and says so."""
+    import zinfer_b200 as z
+    prompt = helpers.random_tokens(1, 3 * page + 9, 256)
+    feed = np.random.default_rng(2).integers(0, 256, size=(290, 6)).tolist()
+    runs = []
+    for prepared in (True, False):
+        engine = shared_always(z.Engine(z.load(model_folders[name], dtype=dtype), max_batch=6, max_seq_len=512, page_size=page))
+        engine.MIN_SHARE_SAVED = 0.41 if page == 64 else 0.15        # some 200 tokens on the answers' own keys outweigh the prompt
+        s, = engine.start(1)
+        engine.step([s], [prompt])
+        slots = [s, *engine.fork(s, 5)]
+        first = engine.length(s) + 1
+        if prepared:
+            with pytest.raises(RuntimeError, match="with these shared prefixes"):
+                engine.prepare_decode(6, first, first + 150, slots=slots)
+        engine.decode(slots, feed[0])
+        if prepared:
+            with pytest.raises(RuntimeError, match="without shared prefixes"):
+                engine.prepare_decode(6, first, first + 150)
+            with pytest.raises(ValueError):
+                engine.prepare_decode(5, first, first + 150, slots=slots)
+            engine.prepare_decode(6, first + 1, first + 150, slots=slots)
+            before = engine.graph_captures
+            assert before >= 2                                        # own keys up to 128, and up to 192
+        out = []
+        for i in range(1, 290):
+            x = engine.decode(slots, feed[i], check=i % 50 == 0)
+            if prepared and i == 150:
+                assert engine.graph_captures == before                # every step of the range was there
+            if i % 17 == 0:
+                out.append(x.cpu().numpy().copy())
+        assert not engine.shared_prefixes(slots) and engine._decode_batches[6].warmed
+        if prepared:
+            engine.prepare_decode(6, first + 290, first + 292, slots=slots)      # by now they share nothing that pays
+        engine.check_status()
+        runs.append(out)
+    for got, want in zip(*runs):
+        assert np.array_equal(got, want)
+
+
 def test_sharing_is_used_where_it_pays(model_folders):
     import zinfer_b200 as z
     engine = z.Engine(z.load(model_folders["tiny_d"], dtype="bf16"), max_batch=10, max_seq_len=1000, page_size=64)

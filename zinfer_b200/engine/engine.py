@@ -173,7 +173,7 @@ class Engine:
         self._host_ring, self._host_next = None, 0      # pinned buffers the sampled tokens are read into
         self._copy_stream = None                        # the stream on which recorded steps' tokens are fetched
         self._takes_prefixes = any(getattr(p, "takes_prefixes", False) for p in model.all_parts())
-        self._ran_shared: set = set()
+        self._ran_shared: set = set()                   # batch sizes and prefixes of which a step has run outside a recording
         self._sharing = (None, [])                      # (slots and the cache's version, what they share): asked for every step
         self.interrupt = threading.Event()   # set it (from a signal handler, another thread, a callback) to end `generate`
         self.stats = None
@@ -204,8 +204,9 @@ class Engine:
     # launches more to record.
     MIN_KEYS_SAVED, MIN_SHARE_SAVED = 4096, 0.25
 
-    def shared_prefixes(self, slots: Sequence[int]) -> list:
-        """[(rows, positions)] as `CacheManager.shared_prefixes`, or [] where reading it once would not pay."""
+    def shared_prefixes(self, slots: Sequence[int], grown: int = 0) -> list:
+        """[(rows, positions)] as `CacheManager.shared_prefixes`, or [] where reading it once would not pay once every sequence has
+        grown by `grown` tokens."""
         if not self._takes_prefixes:
             return []
         key = (tuple(slots), self.cache.sharing_version)
@@ -215,7 +216,7 @@ class Engine:
         if not groups:
             return []
         saved = sum((len(rows) - 1) * keys for rows, keys in groups)
-        every = sum(int(self.cache.lengths[s]) + 1 for s in slots)
+        every = sum(int(self.cache.lengths[s]) + 1 + grown for s in slots)
         return groups if saved >= self.MIN_KEYS_SAVED and saved >= self.MIN_SHARE_SAVED * every else []
 
     @staticmethod
@@ -406,33 +407,47 @@ class Engine:
                 return _PendingTokens(self, batch.host_ring[slot], done)
         return None
 
-    def _decode_graph(self, batch: _DecodeBatch, B: int, longest: int, prefixes=None, longest_own: int = 0) -> torch.Tensor:
-        ctx = StepContext(self.dtype, self.device, self.status, batch.meta_dev, B, B, [1] * B, longest,
-                          memo=batch.memo, sm_count=self.sm_count, prefixes=prefixes,
-                          longest_own=kernels.own_capacity(longest_own))
-        batch.steps += 1            # the kernels run once below (a recording in between runs nothing)
-        if not batch.warmed and prefixes is None:
-            batch.warmed = True
+    def _single_token_ctx(self, batch: _DecodeBatch, longest: int, prefixes, longest_own: int) -> StepContext:
+        return StepContext(self.dtype, self.device, self.status, batch.meta_dev, batch.n_seqs, batch.n_seqs, [1] * batch.n_seqs, longest,
+                           memo=batch.memo, sm_count=self.sm_count, prefixes=prefixes, longest_own=kernels.own_capacity(longest_own))
+
+    def _recording_key(self, n_seqs: int, longest: int, prefixes, longest_own: int) -> tuple:
+        """With prefixes the recording reads the description; what it bakes in is the shape of the launches."""
+        key = self.decode_key(n_seqs, longest)
+        return key if prefixes is None else key + ("shared", prefixes.key(longest_own))
+
+    @staticmethod
+    def _loaded(prefixes) -> tuple:
+        """What a step with these prefixes has loaded and memoised, whatever its lengths: the kernels go by groups and prefixes."""
+        n_seqs, _, groups = prefixes.key(1)
+        return n_seqs, groups
+
+    def _record(self, key: tuple, ctx: StepContext, batch: _DecodeBatch) -> "torch.cuda.CUDAGraph":
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=self._graph_pool):
             self._forward_single_tokens(ctx, batch)
-            return batch.logits
-        key = self.decode_key(B, longest)
-        if prefixes is not None:        # the recording reads the description; what it bakes in is the shape of the launches
-            key += ("shared", prefixes.key(longest_own))
-            # A first step outside a recording loads the kernels that these launches need (and makes what the parts memoise):
-            # neither this nor a step without shared prefixes does it for the other.
-            if key not in self._ran_shared:
+        self._graphs[key] = graph
+        self.graph_captures += 1
+        return graph
+
+    def _decode_graph(self, batch: _DecodeBatch, B: int, longest: int, prefixes=None, longest_own: int = 0) -> torch.Tensor:
+        ctx = self._single_token_ctx(batch, longest, prefixes, longest_own)
+        batch.steps += 1            # the kernels run once below (a recording in between runs nothing)
+        # A first step outside a recording loads the kernels that these launches need (and makes what the parts memoise): neither a
+        # step with shared prefixes nor one without does it for the other.
+        if not batch.warmed if prefixes is None else self._loaded(prefixes) not in self._ran_shared:
+            if prefixes is None:
+                batch.warmed = True
+            else:
                 if len(self._ran_shared) >= 1024:
                     self._ran_shared.clear()
-                self._ran_shared.add(key)
-                self._forward_single_tokens(ctx, batch)
-                return batch.logits
+                self._ran_shared.add(self._loaded(prefixes))
+            self._forward_single_tokens(ctx, batch)
+            return batch.logits
+        key = self._recording_key(B, longest, prefixes, longest_own)
         graph = self._graphs.get(key)
         if graph is None:
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, pool=self._graph_pool):
-                self._forward_single_tokens(ctx, batch)
-            self._graphs[key] = graph
-            self.graph_captures += 1
+            graph = self._record(key, ctx, batch)
             while len(self._graphs) > self.MAX_GRAPHS:
                 self._graphs.popitem(last=False)
         else:
@@ -440,34 +455,42 @@ class Engine:
         graph.replay()
         return batch.logits
 
-    def prepare_decode(self, n_seqs: int, first: int, last: int) -> None:
+    def prepare_decode(self, n_seqs: int, first: int, last: int, slots: Optional[Sequence[int]] = None) -> None:
         """Records, ahead of time, the single-token steps that `n_seqs` sequences need while their
         longest grows from `first` to `last` tokens (one per launch key on the way), so that none of
-        those steps pays for a recording.  Needs one unrecorded step of that batch size to have run."""
+        those steps pays for a recording.  `slots`: the sequences, which may share prefixes (all of them
+        grow by the same number of tokens); without it the steps are those of sequences that share nothing.
+        Needs one unrecorded step of that batch size, with the same prefixes, to have run."""
+        if slots is not None and len(slots) != n_seqs:
+            raise ValueError(f"{len(slots)} slots for a step of {n_seqs} sequences")
         if not self.use_graphs:
             return
         batch = self._decode_batch(n_seqs)
-        if not batch.warmed:
-            raise RuntimeError(f"no single-token step of {n_seqs} sequences has run yet")
+        lengths = [] if slots is None else [int(self.cache.lengths[s]) for s in slots]
         longest = max(first, last)
         length = max(1, first)
+
+        def step_at(length: int) -> tuple:
+            """(prefixes, the most own keys) of the step whose longest sequence has `length` tokens, its own among them."""
+            grown = length - max(lengths, default=0) - 1
+            groups = self.shared_prefixes(slots, grown) if slots else []
+            return (batch.share(groups), self._longest_own(groups, [n + 1 + grown for n in lengths])) if groups else (None, 0)
+
         while True:
-            key = self.decode_key(n_seqs, length)
+            step = step_at(length)
+            if not batch.warmed if step[0] is None else self._loaded(step[0]) not in self._ran_shared:
+                raise RuntimeError(f"no single-token step of {n_seqs} sequences {'with these' if step[0] else 'without'} shared prefixes "
+                                   "has run yet")
+            key = self._recording_key(n_seqs, length, *step)
             if key not in self._graphs:
-                ctx = StepContext(self.dtype, self.device, self.status, batch.meta_dev, n_seqs, n_seqs, [1] * n_seqs,
-                                  length, memo=batch.memo, sm_count=self.sm_count)
-                graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph, pool=self._graph_pool):
-                    self._forward_single_tokens(ctx, batch)
-                self._graphs[key] = graph
-                self.graph_captures += 1
+                self._record(key, self._single_token_ctx(batch, length, *step), batch)
             if length >= longest:
                 break
             # the next length at which some mixer's key may change: keys are functions of coarse
             # buckets, so doubling steps with a linear probe in between find every one of them
             nxt = length + 1
-            while nxt < longest and self.decode_key(n_seqs, nxt) == key:
-                nxt = min(longest, nxt + max(1, nxt // 8))
+            while nxt < longest and self._recording_key(n_seqs, nxt, *step_at(nxt)) == key:
+                nxt = min(longest, nxt + max(1, (step_at(nxt)[1] or nxt) // 8))
             length = nxt
         while len(self._graphs) > self.MAX_GRAPHS:
             self._graphs.popitem(last=False)
