@@ -2184,6 +2184,9 @@ def _shared_call(q, k_cache, v_cache, seq_start, seq_slot, page_table, shared, n
     for t in (k_cache, v_cache, seq_start, seq_slot, page_table, sink, gate, shared.words):
         if t is not None and t.device != q.device:
             raise KernelError(f"attention_shared: tensors of {q.device} and {t.device}")
+    most = max((keys for _, keys in shared.groups), default=0)
+    if most > page_table.shape[1] * page_size:      # (a group's walk would read on behind its first row's page numbers)
+        raise KernelError(f"attention_shared: {most} shared keys, but a sequence has {page_table.shape[1]} pages of {page_size} at most")
     G, dt = n_heads // n_kv, dtype_code(q.dtype)
     pairs = G * max((rows for rows, _ in shared.groups), default=1)
     longest = max((prefix_capacity(keys) for _, keys in shared.groups), default=0)
