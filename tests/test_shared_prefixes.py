@@ -155,3 +155,16 @@ def test_the_tensor_cores_take_what_they_take_without_shared_prefixes():
                     code = k.dtype_code(dtype)
                     tile = k._fn("attention_shared", "zk_attn_shared_tile_rows")(code, heads // n_kv, width, width, page, 200, 9000)
                     assert tile == (128 if alone else 32)
+
+
+def test_a_status_word_of_another_device_is_refused(monkeypatch):
+    """A kernel would write through an address that is none on its own device."""
+    import torch
+    word = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(k.KernelError, match="CUDA"):
+        k._need_status(word, torch.device("cuda", 0))
+    monkeypatch.setattr(k, "_need", lambda *args, **kw: None)          # from here on the CPU stands for a second device
+    k._need_status(word, torch.device("cpu"))
+    for bad, device in ((word, torch.device("cuda", 0)), (word[:0], torch.device("cpu"))):
+        with pytest.raises(k.KernelError, match="expected one"):
+            k._need_status(bad, device)

@@ -268,6 +268,13 @@ def _need_here(t: torch.Tensor, what: str) -> None:
         raise KernelError(f"{what}: tensors of {t.device}, but the current device is cuda:{_raw_device()}")
 
 
+def _need_status(status: torch.Tensor, device: torch.device) -> None:
+    """A status word that a kernel on `device` may write."""
+    _need(status, "status", torch.int32)
+    if status.numel() == 0 or status.device != device:
+        raise KernelError(f"status: {status.numel()} words on {status.device}, expected one on {device}")
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DT[dtype]
@@ -2142,7 +2149,7 @@ def attention_shared(q, k_cache, v_cache, seq_start, seq_slot, page_table, share
     if status is None:
         status = status_word(q.device)
     else:
-        _need(status, "status", torch.int32)
+        _need_status(status, q.device)
     out = q.new_empty((shared.n_seqs, width))
     part_ml = torch.empty(floats, dtype=torch.float32, device=q.device)
     at = part_ml.data_ptr()
@@ -2338,7 +2345,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     n, V, ld, dt, sms = call
     _need_here(logits, "token_logprobs")
     if status is not None:
-        _need(status, "status", torch.int32)
+        _need_status(status, logits.device)
     floats = logits if logits.dtype is torch.float32 else torch.empty(0, dtype=torch.float32, device=logits.device)
     r = TokenLogprobs(floats.new_empty(n), tokens.new_empty(n), floats.new_empty(n), tokens.new_empty((n, top)),
                       floats.new_empty((n, top)))
