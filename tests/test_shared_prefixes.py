@@ -168,3 +168,16 @@ def test_a_status_word_of_another_device_is_refused(monkeypatch):
     for bad, device in ((word, torch.device("cuda", 0)), (word[:0], torch.device("cpu"))):
         with pytest.raises(k.KernelError, match="expected one"):
             k._need_status(bad, device)
+
+
+def test_every_code_of_the_shared_kernel_has_a_text_that_names_it():
+    """A wait that gives up, a short row, a missing page: what the engine raises says where it may have come from."""
+    import re
+    from pathlib import Path
+
+    from zinfer_b200.engine.engine import _STATUS_TEXT
+    source = (Path(k.__file__).parent / "csrc" / "attention_shared.cu").read_text()
+    waits = {int(c) for c in re.findall(r"wait\(&?\w+(?:\[[^\]]*\])?, [^;\n]*?, (\d+)\)", source)}
+    assert waits == {13, 14, 15, 16, 17, 18}
+    assert all("shared prefix" in _STATUS_TEXT[c] for c in waits)
+    assert {int(c) for c in re.findall(r"atomicExch\(a\.status, (\d+)\)", source)} == {2, 20} <= set(_STATUS_TEXT)

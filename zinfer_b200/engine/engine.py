@@ -31,12 +31,12 @@ class StepError(RuntimeError):
 _STATUS_TEXT = {1: "a token id lies outside the vocabulary", 2: "a token's position has no cache page",
                 11: "a tensor-core contraction gave up waiting for a free pipeline stage",
                 12: "a tensor-core contraction gave up waiting for its operand tiles",
-                13: "a tensor-core contraction gave up waiting for its accumulator",
-                14: "the tcgen05 prompt attention gave up waiting for a free K/V stage",
-                15: "the tcgen05 prompt attention gave up waiting for its query or K/V tiles",
-                16: "the tcgen05 prompt attention gave up waiting for the probabilities",
-                17: "the tcgen05 prompt attention gave up waiting for the scores",
-                18: "the tcgen05 prompt attention gave up waiting for P V",
+                13: "a tensor-core contraction gave up waiting for its accumulator, or tcgen05 attention of a shared prefix for a score buffer",
+                14: "tcgen05 attention (of a prompt, or of a shared prefix) gave up waiting for a free K/V stage",
+                15: "tcgen05 attention (of a prompt, or of a shared prefix) gave up waiting for its query or K/V tiles",
+                16: "tcgen05 attention (of a prompt, or of a shared prefix) gave up waiting for the probabilities",
+                17: "tcgen05 attention (of a prompt, or of a shared prefix) gave up waiting for the scores",
+                18: "tcgen05 attention (of a prompt, or of a shared prefix) gave up waiting for P V",
                 19: "the gated delta rule gave up waiting for a chunk's vectors",
                 20: "a sequence is shorter than the prefix it shares"}
 
