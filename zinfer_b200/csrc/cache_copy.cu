@@ -12,6 +12,7 @@
 // numbers in 6 calls: 41 us for 234 MB, nearly all of it written.
 #include "common.cuh"
 #include <algorithm>
+#include <atomic>
 #include <new>
 
 namespace {
@@ -116,6 +117,17 @@ __global__ void __launch_bounds__(THREADS) cache_copy_kernel(const __grid_consta
 
 }  // namespace
 
+// The current device's SMs, asked for once per device.
+static int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 1;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 extern "C" {
 
 // What a copy must not be given, since it would leave the tensors: 1: an entry outside; 2: a count outside.  Host only.
@@ -182,11 +194,11 @@ int zk_cache_copy(const void* tensors, int n_tensors, const int* src, const int*
         most = std::max(most, e[4] * e[6] * (((long long)a.most_count * e[7] + PIECE - 1) / PIECE));
       }
       // Runs of copies of one entry: where that still leaves four blocks per SM.  63 copies of 41 tokens and of a state of
-      // 6 x 512 KB: 43.0 us in runs of four (43.4 of eight, 46.7 of sixteen), 47.2 one by one; 512 pages that are copied once
-      // 145 and 128.
+      // 6 x 512 KB when this was chosen: 43.0 us in runs of four (43.4 of eight, 46.7 of sixteen), 47.2 one by one; 512 pages that are
+      // copied once 145 and 128.
       int follow = 0;
       for (int i = 1; i < nm; ++i) follow += a.src[i] == a.src[i - 1] && a.count[i] == a.count[i - 1];
-      const bool spread = 4 * follow >= 3 * (nm - 1) && most * (nm / 4) >= 4 * 148;
+      const bool spread = 4 * follow >= 3 * (nm - 1) && most * (nm / 4) >= 4LL * sm_count();
       const dim3 grid((unsigned)std::min(most * (spread ? (nm + 3) / 4 : nm), 1LL << 30), 1, nt);
       const int rc = spread ? zk_launch_dependent(cache_copy_kernel<4>, grid, dim3(THREADS), 0, stream, a)
                             : zk_launch_dependent(cache_copy_kernel<1>, grid, dim3(THREADS), 0, stream, a);
