@@ -54,7 +54,7 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--xtc-min-keep", type=int, default=1)
     g.add_argument("--seed", type=int, default=None, help="RNG seed (default: time)")
     ap.add_argument("--samples", type=int, default=1, metavar="N",
-                    help="answers to every prompt: it is run once and forked (default 1)")
+                    help="answers to every prompt, which each batch of them runs once and forks (default 1)")
     ap.add_argument("--logprobs", type=int, default=None, metavar="K",
                     help="print every token's log probability, rank and the K most likely tokens (0 to 32)")
     ap.add_argument("--score", action="store_true",

@@ -163,7 +163,7 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // K padded by 16 bytes), then RT rows x 4 values of every 64 of the result; threads without a row skip the arithmetic.  K and V
 // lie in shared memory in their own type, two tiles of each: the next one is brought in by cp.async while this one is worked
 // on, four threads to a row, so that no address needs a division (with loads that waited, a tile took some 5 us; 13 rows of
-// 16 heads behind 900 to 2,500 keys, float32: 43 us a call then, 20 now).  Bound by reading K and V from shared memory, every warp all of a
+// 16 heads behind 900 to 2,500 keys, float32: 43 us a call then, 17 now).  Bound by reading K and V from shared memory, every warp all of a
 // tile: 2.7 us of a tile's 6 are its scores' (at two blocks an SM).
 constexpr int GK = 64, G_THREADS = 256;
 

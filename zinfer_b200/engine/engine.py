@@ -540,7 +540,8 @@ class Engine:
     def generate(self, prompts, max_new_tokens: int = 256, sampling=None, stop_ids=None, on_step=None,
                  samples: Optional[int] = None, logprobs: Optional[int] = None, **sampling_options):
         """Generates for every prompt (a list of token ids each); returns a GenerationResult per
-        prompt, in order.  `samples`: so many answers to every prompt, which is run once and forked; the result is then a list of
+        prompt, in order.  `samples`: so many answers to every prompt, which each batch of them runs once and forks (a batch holds as
+        many answers as there are slots, and as the cache would hold with a prompt each); the result is then a list of
         GenerationResults per prompt (answer j to prompt i is request i * samples + j: it draws its own random numbers).  `logprobs`:
         every result also tells, in `logprobs`, its tokens' log probabilities under the model (before penalties and
         temperature), their ranks, the entropies and that many alternatives (0 to 32).  `sampling` is a SamplingParams, or give its fields as keyword
