@@ -1309,12 +1309,12 @@ int launch_merge(const SharedArgs& a, cudaStream_t stream) {
 extern "C" {
 
 // (sequence, head) pairs that one block's tile of a group holds; `pairs`: the most pairs a group has, `longest`: the keys of the longest
-// prefix.  Tiles of 32, 64 and 128 are the tcgen05 kernel's, tiles of 16 the mma.sync one's (both: bfloat16 heads of 64 or 128, at most
-// 16 to a KV head, and pages of whole key tiles).  A tile of 16 costs less to start, so it serves groups that fit one, unless their keys
-// are many, and few keys of two (8 KV heads, one group, us): heads of 64, tiles of 16 / 32: 8 pairs behind 1,024 keys 5.9 / 7.5, behind 4,096 9.5 / 8.9, 16
-// pairs 6.9 / 7.8, 11.2 / 9.1, 32 behind 256 7.7 / 7.8, behind 1,024 9.1 / 8.3; heads of 128, tiles of 16 / 64: 8 pairs 7.3 / 8.4,
-// 12.0 / 10.1, 16 behind 256 9.3 / 8.2.  Smaller tcgen05 tiles share a row's keys out over more warps: six groups of 32 pairs behind
-// 16,384 keys, tiles of 32 / 64 / 128: heads of 64 40 / 40 / 52, behind 4,096 16.4 / 17.2 / 20.9, of 128 25.9 / 25.4 / 26.5 there.
+// prefix.  Tiles of 32, 64 and 128 are the tcgen05 kernel's, tiles of 16 the mma.sync one's (both: bfloat16 heads of 64 or 128, at most 16
+// to a KV head, and pages of whole key tiles).  A tile of 16 costs less to start, so it serves groups that fit one, unless their keys are
+// many, and few keys of two (8 KV heads, one group, us): heads of 64, tiles of 16 / 32: 8 pairs behind 1,024 keys 5.9 / 7.5, behind 4,096
+// 9.5 / 8.9, 16 pairs 6.9 / 7.8, 11.2 / 9.1, 32 behind 256 7.7 / 7.8, behind 1,024 9.1 / 8.3; heads of 128, tiles of 16 / 64: 8 pairs 7.3
+// / 8.4, 12.0 / 10.1, 16 behind 256 9.3 / 8.2.  Smaller tcgen05 tiles share a row's keys out over more warps: six groups of 32 pairs
+// behind 16,384 keys, tiles of 32 / 64 / 128: heads of 64 40 / 40 / 52, behind 4,096 16.4 / 17.2 / 20.9, of 128 25.9 / 25.4 / 26.5 there.
 // Other types and heads: 32 rows a block on FMAs, 16 where that holds all.
 int zk_attn_shared_tile_rows(int dtype, int G, int hd, int vd, int page_size, int pairs, int longest) {
   if (!mma_takes(dtype, G, hd, vd, page_size)) return pairs > 16 ? 32 : 16;
